@@ -7,6 +7,7 @@ from collections import namedtuple
 
 import torch
 from torch.autograd import Function
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _lib
 
@@ -104,9 +105,10 @@ def log_probs(logits, ids=None, top=0, dim=-1):
       top_log_prob, top_ids   [..., top]: the ``top`` (<= 64) likeliest categories and their log probabilities, the lowest index first among
                     equal logits; None for top = 0
 
-    All but top_ids carry gradients (first order).  ``ids`` (int32 / int64) has the shape of ``logits`` without ``dim``; so have the results.  The
-    rows may lie apart (a channel slice, ``dim=1`` of a channels_last [N, D, H, W] tensor): read in place where they are equally
-    spaced with contiguous categories, else from one copy.  A row whose logits are all -inf has lse and log probabilities -inf,
+    All but top_ids carry gradients (first order, reverse mode; a forward-mode dual tensor is refused).  ``ids`` (int32 / int64) has
+    the shape of ``logits`` without ``dim``; so have the results.  The rows may lie apart (a channel slice, ``dim=1`` of a
+    channels_last [N, D, H, W] tensor): read in place where they are equally spaced with contiguous categories, else from one
+    copy.  A row whose logits are all -inf has lse and log probabilities -inf,
     entropy 0 and gradient 0; NaN or +inf in a row makes its values NaN."""
     if not logits.is_cuda:
         raise RuntimeError("logits must be a CUDAtensor ")
@@ -126,7 +128,8 @@ def log_probs(logits, ids=None, top=0, dim=-1):
             raise RuntimeError(f"log_probs: ids must be an int32 / int64 tensor of shape {tuple(x.shape[:-1])} on {logits.device} "
                                f"(found {ids.dtype} {tuple(ids.shape)} on {ids.device})")
         ids = ids.contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
+    # (a dual tensor, which stays one under no_grad, takes the function too: that raises for want of a jvp; the kernel would drop the tangent)
+    if (logits.requires_grad and torch.is_grad_enabled()) or unpack_dual(logits).tangent is not None:
         return LogProbs(*_lib.apply_function(LogProbsFunction, x, ids, top))
     x, rows, R = _rows(x)
     return LogProbs(*_forward(x, ids, top, rows, R)[:5])
