@@ -144,7 +144,8 @@ class TrainStep(nn.Module):
                 if isinstance(m, (nn.Conv2d, nn.ConvTranspose2d)):
                     m.to(memory_format=torch.channels_last)
         # cfg["depth_loss"]: "bce" (default: the reference's binary cross entropy on the distribution, exps/mm_training_aim.py:165-178) or "nll", the
-        # negative log probability of the label's bin from the logits (get_depth_nll); cfg["optimizer_states"]: "32bit" (default) or "8bit" (dp/optim8.py)
+        # negative log probability of the label's bin from the logits, over the pixels with a LiDAR return (get_depth_nll);
+        # cfg["optimizer_states"]: "32bit" (default) or "8bit" (dp/optim8.py)
         self.depth_loss_kind, self.optimizer_states = cfg.get("depth_loss", "bce"), cfg.get("optimizer_states", "32bit")
         if self.depth_loss_kind not in ("bce", "nll") or self.optimizer_states not in ("32bit", "8bit"):
             raise ValueError(f"TrainStep: depth_loss {self.depth_loss_kind!r} (bce | nll), optimizer_states {self.optimizer_states!r} (32bit | 8bit)")
@@ -298,11 +299,15 @@ class TrainStep(nn.Module):
         return 3.0 * (bce * fg).sum() / fg.sum().clamp(min=1.0)
 
     def get_depth_nll(self, depth_labels, depth_logits):
-        """The categorical form of the depth loss: 3 x the mean negative log probability of the label's bin over the pixels that have a label (the same
-        foreground rule and weight as get_depth_loss), from the logits [B*N, D, fH, fW] -- finite where the distribution's fp32
-        probabilities have underflowed and BCE's gradient with them."""
-        value, ids = depth_labels.max(1)
-        fg = value > 0.0
+        """The categorical form of the depth loss: 3 x the mean negative log probability of the label's bin over the pixels that have a label, from the
+        logits [B*N, D, fH, fW] -- finite where the distribution's fp32 probabilities have underflowed and BCE's gradient with them.
+        depth_labels: the int bins of ops/train_targets.py's depth_labels, in which 0 is a pixel without a return in range (a depth in range has
+        bin 1 or more) and so has no label here; or rows of D, one-hot, where a row of zeros has none."""
+        if depth_labels.dim() == 1:
+            fg, ids = depth_labels > 0, depth_labels
+        else:
+            value, ids = depth_labels.max(1)
+            fg = value > 0.0
         n, _, fH, fW = depth_logits.shape
         log_prob = log_probs(depth_logits, torch.where(fg, ids, -1).view(n, fH, fW), dim=1).log_prob
         return -3.0 * log_prob.sum() / fg.sum().clamp(min=1)
@@ -313,7 +318,7 @@ class TrainStep(nn.Module):
 
     def forward_loss(self, batch):
         sweep_imgs, mats, pointclouds, gt_boxes, gt_labels = batch
-        depth_labels_flat = input_depth = None
+        depth_labels_flat = depth_bins = input_depth = None
         if self.use_cam:
             # training_step :256-259 in two launch sequences: the flags are drawn like augment_images draws them (:98), then
             #   get_depth_labels + the label half of augment_images   -> mmt_depth_labels_flipped (mirrored label write)
@@ -324,7 +329,9 @@ class TrainStep(nn.Module):
             flips = np.random.uniform(size=(B * S * N)) > 0.5 if self.augment else np.zeros((B * S * N), dtype=bool)
             fl = camera_flags_to_device(flips, sweep_imgs.device)
             depth_labels_flat = depth_labels(pointclouds, mats["extrinsics"][:, 0], mats["intrin_mats"][:, 0], mats["bda_mat"],
-                                             (H, W), self.downsample, self.dbound, self.depth_channels, flipped=fl)
+                                             (H, W), self.downsample, self.dbound, self.depth_channels, return_bins=self.depth_loss_kind == "nll", flipped=fl)
+            if self.depth_loss_kind == "nll":
+                depth_labels_flat, depth_bins = depth_labels_flat            # (its one-hot rows are never empty: without a return they name bin 0)
             sweep_imgs = normalize_flip_images(sweep_imgs, IMG_MEAN, IMG_STD, fl,
                                                channels_last=os.environ.get("MMT_MEMORY_FORMAT", "channels_last") == "channels_last")
             mats = dict(mats, flipped=fl)                    # :258 (the batch's own dict is left alone)
@@ -338,7 +345,7 @@ class TrainStep(nn.Module):
         detection_loss = self.model.loss(targets, preds)
         depth_loss = detection_loss.new_zeros(())
         if self.use_cam:
-            depth_loss = (self.get_depth_nll if self.depth_loss_kind == "nll" else self.get_depth_loss)(depth_labels_flat, depth_preds)
+            depth_loss = self.get_depth_nll(depth_bins, depth_preds) if self.depth_loss_kind == "nll" else self.get_depth_loss(depth_labels_flat, depth_preds)
         return detection_loss + depth_loss, detection_loss, depth_loss
 
     def _gradient_streams(self):
