@@ -5,11 +5,13 @@ instead of 28.  Tensors of fewer than ``min_8bit_size`` elements keep 32-bit mom
 Further than ClipAdamW it takes bf16 parameters (rounded stochastically: no fp32 copy is needed for small updates to count), several
 parameter groups under one clipping norm, and parameters that join later (every one has its own step count).
 """
+import itertools
 import math
 import operator
 
 import numpy as np
 import torch
+from torch._C._dynamo.guards import TensorGuards
 
 from .. import _lib
 from .optim import RING, _dense, _same_layout
@@ -17,8 +19,7 @@ from .optim import RING, _dense, _same_layout
 BLOCK = 32          # elements that share a scale byte
 ALIGN = 256         # every tensor's moments begin at a multiple of this many elements of the state buffers
 COLUMNS = 9         # MMT_ADAMW8_COLUMNS
-_GRAD, _DTYPE = operator.attrgetter("grad"), operator.attrgetter("dtype")           # (for map: a step asks every parameter)
-_ADDRESS, _CONTIGUOUS, _NUMEL = torch.Tensor.data_ptr, torch.Tensor.is_contiguous, torch.Tensor.numel
+_GRAD, _ADDRESS, _NUMEL = operator.attrgetter("grad"), torch.Tensor.data_ptr, torch.Tensor.numel           # (for map: a step asks every parameter)
 STEP_ROW = np.dtype([("grad", "<i8"), ("h", "<f4", (8,))])
 
 
@@ -32,6 +33,12 @@ def _mix(x):
 
 def _codes_dtype(second):
     return torch.float8_e5m2 if second else torch.float8_e4m3fn
+
+
+def _as_now(tensors):
+    """An object whose ``check(*tensors)`` says whether size, strides, type and device of every tensor are what they are now: one call for all of
+    them (separate questions, one Python call a tensor each, would cost as much as a small step's launches).  Holds no tensor."""
+    return TensorGuards(*tensors, dynamic_dims_sizes=[list(t.shape) for t in tensors], dynamic_dims_strides=[list(t.stride()) for t in tensors])
 
 
 def _memory_order(t):
@@ -245,13 +252,11 @@ class ClipAdamW8(torch.optim.Optimizer):
             slots.append(dict(host=host, rows=host.numpy().view(STEP_ROW), device=torch.empty(host.numel(), dtype=torch.uint8, device=dev),
                               partials=torch.empty(partials, dtype=torch.float64, device=dev),
                               norm=torch.zeros(2, dtype=torch.float32, device=dev), event=None))
-        others = [i for i, p in enumerate(ps) if not p.is_contiguous()]
         group_of = {p: gi for gi, g in enumerate(self.param_groups) for p in g["params"]}
         self._plan = dict(ps=ps, addresses=addresses, n_chunks=n_chunks, chunk=chunk, table=torch.from_numpy(table).to(dev),
                           chunk_t=torch.from_numpy(chunk_t).to(dev), chunk_o=torch.from_numpy(chunk_o).to(dev), slots=slots, turn=0,
                           index=torch.tensor([self._index[p] for p in ps]), group=np.array([group_of[p] for p in ps]),
-                          dtypes=[p.dtype for p in ps], numels=[p.numel() for p in ps], contiguous=[p.is_contiguous() for p in ps], others=lambda seq: [seq[i] for i in others],
-                          strides=[ps[i].stride() for i in others])
+                          dtypes=[p.dtype for p in ps], as_checked=None)
         torch.cuda.current_stream(dev).synchronize()          # (built on this stream, read on whichever stream a step runs on)
         return self._plan
 
@@ -275,30 +280,18 @@ class ClipAdamW8(torch.optim.Optimizer):
                 raise RuntimeError("ClipAdamW8.step() cannot be captured into a graph: gradients' addresses and step counts come from the host")
         ps = self._live
         grads = list(map(_GRAD, ps))
-        try:
-            dtypes = list(map(_DTYPE, grads))
-        except AttributeError:                                # (a parameter without a gradient takes no part)
+        if any(map(operator.is_, grads, itertools.repeat(None))):          # (a parameter without a gradient takes no part)
             ps = [p for p, g in zip(ps, grads) if g is not None]
             grads = [g for g in grads if g is not None]
-            dtypes = list(map(_DTYPE, grads))
         if not ps:
             return loss
         addresses = list(map(_ADDRESS, ps))
         plan = self._plan
         if plan is None or plan["addresses"] != addresses or not (plan["ps"] is ps or all(map(operator.is_, plan["ps"], ps))):
             plan = self._tables(ps, addresses, grads)
-        # the gradients' sizes and layouts: contiguous like the parameter (the quick question), or strides equal to its
-        if (dtypes != plan["dtypes"] or list(map(_NUMEL, grads)) != plan["numels"] or list(map(_CONTIGUOUS, grads)) != plan["contiguous"]
-                or [g.stride() for g in plan["others"](grads)] != plan["strides"]):
-            for i, (p, g) in enumerate(zip(ps, grads)):
-                if p.numel() != plan["numels"][i] or p.dtype != plan["dtypes"][i] or not _same_layout(self.state[p]["exp_avg"], p):
-                    raise RuntimeError("ClipAdamW8: a parameter has changed its size, type or layout in place (its moments have not)")
-                if g.shape != p.shape:
-                    raise RuntimeError(f"ClipAdamW8: a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(p.shape)}")
-                if g.is_sparse:
-                    raise RuntimeError("ClipAdamW8: a gradient is sparse")
-                if g.dtype != p.dtype or not _same_layout(g, p):
-                    grads[i] = p.grad = torch.empty_like(p).copy_(g)
+        # one question for all: is everything as it was when each was last looked at
+        if plan["as_checked"] is None or not plan["as_checked"].check(*ps, *grads):
+            self._check_each(plan, ps, grads)
         with _lib.on_device(dev):
             slot = plan["slots"][plan["turn"]]
             if slot["event"] is not None:
@@ -318,6 +311,26 @@ class ClipAdamW8(torch.optim.Optimizer):
             plan["turn"] = (plan["turn"] + 1) % RING
         self.last_norm = slot["norm"]
         return loss
+
+    def _check_each(self, plan, ps, grads):
+        """Raises unless every parameter is laid out like its moments and has a dense gradient of its shape; gradients of another type or memory order
+        are replaced (in ``grads`` and the parameter) by ones of the parameter's."""
+        replaced = False
+        for i, (p, g) in enumerate(zip(ps, grads)):
+            m = self.state[p]["exp_avg"]
+            # (a contiguous parameter seen through another shape is still in its moments' order)
+            if p.dtype != plan["dtypes"][i] or p.numel() != m.numel() or not (_same_layout(m, p) or m.is_contiguous() and p.is_contiguous()):
+                raise RuntimeError("ClipAdamW8: a parameter has changed its size, type or layout in place (its moments have not)")
+            if g.shape != p.shape:
+                raise RuntimeError(f"ClipAdamW8: a gradient of shape {tuple(g.shape)} for a parameter of shape {tuple(p.shape)}")
+            if g.is_sparse:
+                raise RuntimeError("ClipAdamW8: a gradient is sparse")
+            if g.device != p.device:
+                raise TypeError("ClipAdamW8: a gradient is elsewhere than its parameter")
+            if g.dtype != p.dtype or not _same_layout(g, p):
+                grads[i] = p.grad = torch.empty_like(p).copy_(g)
+                replaced = True
+        plan["as_checked"] = None if replaced else _as_now(ps + grads)
 
     def _key(self, count):
         return _mix((_mix(self.seed & 0xFFFFFFFF) + count) & 0xFFFFFFFF)
