@@ -122,6 +122,9 @@ class ClipAdamW8(torch.optim.Optimizer):
                 self.param_groups.pop()
                 raise
 
+    def _packed(self, p):
+        return p.numel() >= self.min_8bit_size
+
     # ---- the state buffers: one allocation per kind, every parameter's moments a view
     def _layout(self):
         """Gives every parameter its place in new state buffers (again after a group was added: what is there moves along)."""
@@ -133,11 +136,15 @@ class ClipAdamW8(torch.optim.Optimizer):
                 raise TypeError("ClipAdamW8: the parameters are on several devices")
         for g in self.param_groups:
             self._check_hyper(g)
+        held = {p: st for p, st in self.state.items() if "exp_avg" in st}
+        for p, st in held.items():
+            if not _same_layout(st["exp_avg"], p) or ("exp_avg_scale" in st) != self._packed(p):
+                raise RuntimeError("ClipAdamW8: a parameter has changed its size or layout, and its moments (or min_8bit_size) have not")
         n8 = n32 = 0
         place = {}
         for p in ps:
             size = -(-p.numel() // ALIGN) * ALIGN
-            if p.numel() >= self.min_8bit_size:
+            if self._packed(p):
                 place[p] = (True, n8)
                 n8 += size
             else:
@@ -153,7 +160,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._typed = dict(buffers, exp_avg=buffers["exp_avg"].view(torch.float8_e4m3fn), exp_avg_sq=buffers["exp_avg_sq"].view(torch.float8_e5m2))
         self._counts = torch.zeros(len(ps), dtype=torch.float32)
         self._index = {p: t for t, p in enumerate(ps)}
-        self._fill_state({p: st for p, st in self.state.items() if "exp_avg" in st})
+        self._fill_state(held)
         self._live = [p for p in ps if p.numel()]
         self._empty = [p for p in ps if not p.numel()]
         self._sizes = {p: p.numel() for p in ps}
@@ -378,7 +385,7 @@ class ClipAdamW8(torch.optim.Optimizer):
     def _converted(self, p, st, key):
         """A saved moment in the form and memory order that this parameter keeps it in: {key: codes, key_scale: scales} or {key: fp32}."""
         x, scales, second = st[key].to(p.device), st.get(key + "_scale"), key == "exp_avg_sq"
-        packed = self._place[p][0]
+        packed = self._packed(p)
         if scales is not None:
             x, scales = x.view(_codes_dtype(second)), scales.to(p.device)
             if scales.dtype != torch.uint8 or scales.numel() != -(-x.numel() // BLOCK):
