@@ -125,15 +125,19 @@ class ClipAdamW8(torch.optim.Optimizer):
     def _packed(self, p):
         return p.numel() >= self.min_8bit_size
 
-    # ---- the state buffers: one allocation per kind, every parameter's moments a view
-    def _layout(self):
-        """Gives every parameter its place in new state buffers (again after a group was added: what is there moves along)."""
-        ps = [p for g in self.param_groups for p in g["params"]]
+    @staticmethod
+    def _check_params(ps):
         for p in ps:
             if not (p.is_cuda and p.dtype in (torch.float32, torch.bfloat16) and _dense(p)):
                 raise TypeError("ClipAdamW8 takes dense fp32 / bf16 CUDA parameters")
             if p.device != ps[0].device:
                 raise TypeError("ClipAdamW8: the parameters are on several devices")
+
+    # ---- the state buffers: one allocation per kind, every parameter's moments a view
+    def _layout(self):
+        """Gives every parameter its place in new state buffers (again after a group was added: what is there moves along)."""
+        ps = [p for g in self.param_groups for p in g["params"]]
+        self._check_params(ps)
         for g in self.param_groups:
             self._check_hyper(g)
         held = {p: st for p, st in self.state.items() if "exp_avg" in st}
@@ -359,34 +363,50 @@ class ClipAdamW8(torch.optim.Optimizer):
     # ---- checkpoints
     @torch.no_grad()
     def load_state_dict(self, state_dict):
-        saved = state_dict["state"]
-        for g in state_dict["param_groups"]:
-            self._check_hyper({**self.defaults, **g})
-        order = [k for g in state_dict["param_groups"] for k in g["params"]]
-        if len(order) != len(self._params):
-            raise ValueError("ClipAdamW8: the state is of another number of parameters")
-        for k, p in zip(order, self._params):
-            st = saved.get(k, {})
-            for key in ("exp_avg", "exp_avg_sq"):
-                if key in st and tuple(st[key].shape) != tuple(p.shape):
-                    raise ValueError(f"ClipAdamW8: {key} of shape {tuple(st[key].shape)} for a parameter of shape {tuple(p.shape)}")
-        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})
-        states = {}
-        for k, p in zip(order, self._params):
-            st = saved.get(k, {})
-            if "exp_avg" in st:
-                states[p] = dict(step=st["step"])
-                for key in ("exp_avg", "exp_avg_sq"):
-                    states[p].update(self._converted(p, st, key))
-        self.state.clear()
-        self._layout()                            # (new buffers: the given tensors may be views of the ones there were)
-        self._fill_state(states)
+        """Takes effect whole or not at all: every moment is checked and converted before anything is replaced."""
+        loaded = {}
+
+        def convert(_, sd):                       # last of the pre-hooks: what they made of the state dict is what is loaded
+            saved = sd["state"]
+            for g in sd["param_groups"]:
+                self._check_hyper({**self.defaults, **g})
+            order = [k for g in sd["param_groups"] for k in g["params"]]
+            if len(order) != len(self._params):
+                raise ValueError("ClipAdamW8: the state is of another number of parameters")
+            self._check_params(self._params)
+            for k, p in zip(order, self._params):
+                st = saved.get(k, {})
+                if "exp_avg" in st or "exp_avg_sq" in st:
+                    loaded[p] = self._loaded(p, st)
+            return {**sd, "state": {}}
+
+        def install(_):                           # first of the post-hooks: the rest find the moments there
+            self._layout()                        # (new buffers: the given tensors may be views of the ones there were)
+            self._fill_state(loaded)
+
+        hooks = self.register_load_state_dict_pre_hook(convert), self.register_load_state_dict_post_hook(install, prepend=True)
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _loaded(self, p, st):
+        """A parameter's saved state, in the form that it is kept in here."""
+        for key in ("step", "exp_avg", "exp_avg_sq"):
+            if key not in st:
+                raise ValueError(f"ClipAdamW8: a state without {key}")
+            if key != "step" and tuple(st[key].shape) != tuple(p.shape):
+                raise ValueError(f"ClipAdamW8: {key} of shape {tuple(st[key].shape)} for a parameter of shape {tuple(p.shape)}")
+        return dict(step=float(st["step"]), **self._converted(p, st, "exp_avg"), **self._converted(p, st, "exp_avg_sq"))
 
     def _converted(self, p, st, key):
         """A saved moment in the form and memory order that this parameter keeps it in: {key: codes, key_scale: scales} or {key: fp32}."""
         x, scales, second = st[key].to(p.device), st.get(key + "_scale"), key == "exp_avg_sq"
         packed = self._packed(p)
         if scales is not None:
+            if x.element_size() != 1:
+                raise ValueError(f"ClipAdamW8: {key} is {x.dtype} beside its scales, not in 8 bits")
             x, scales = x.view(_codes_dtype(second)), scales.to(p.device)
             if scales.dtype != torch.uint8 or scales.numel() != -(-x.numel() // BLOCK):
                 raise ValueError(f"ClipAdamW8: {key}_scale does not fit {key}")
