@@ -86,8 +86,9 @@ class ClipAdamW8(torch.optim.Optimizer):
     State of a parameter: ``step`` and, from min_8bit_size elements on, ``exp_avg`` (float8_e4m3fn), ``exp_avg_sq`` (float8_e5m2) in the
     parameter's shape and memory order with ``exp_avg_scale``, ``exp_avg_sq_scale`` (uint8 per 32 elements, see pack_moment); fp32 moments
     below.  The update itself uses unrounded moments; what is stored is rounded stochastically by bits that are a function of ``seed``, the
-    largest step count among the parameters that take part (one of them may have joined late: its own would bring the bits of an
-    earlier step back) and the element's position, so a run repeats exactly and ranks of a data-parallel job agree.
+    element's position and the step's draw: one more than the largest that any parameter taking part has had (``draw`` in its state), so a run repeats
+    exactly, ranks of a data-parallel job agree, and a parameter never meets the bits of an earlier step again, whoever joins or
+    leaves.  (Parameters that have taken part in every step: the step count.)
 
     ``state_dict()`` resumes exactly (with the same ``seed``).  ``load_state_dict`` also takes the state of torch.optim.AdamW or ClipAdamW (32-bit moments are packed), and
     ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of the last step on the device.
@@ -162,7 +163,7 @@ class ClipAdamW8(torch.optim.Optimizer):
                        exp_avg_32=f32(n32), exp_avg_sq_32=f32(n32))
         self._buffers, self._place, self._params, self._n8 = buffers, place, ps, n8
         self._typed = dict(buffers, exp_avg=buffers["exp_avg"].view(torch.float8_e4m3fn), exp_avg_sq=buffers["exp_avg_sq"].view(torch.float8_e5m2))
-        self._counts = torch.zeros(len(ps), dtype=torch.float32)
+        self._counts, self._draws = torch.zeros(len(ps), dtype=torch.float32), torch.zeros(len(ps), dtype=torch.int64)
         self._index = {p: t for t, p in enumerate(ps)}
         self._fill_state(held)
         self._live = [p for p in ps if p.numel()]
@@ -173,7 +174,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         """The parameters' moments and step counts from other tensors of the same form, in the same memory order."""
         to, source = {1: [], 4: []}, {1: [], 4: []}           # by element size: one copy for all the codes and scales, one for all the fp32 moments
         for p, st in states.items():
-            self._give_state(p, float(st["step"]))
+            self._give_state(p, float(st["step"]), int(st["draw"]))
             packed, at = self._place[p]
             for key in ("exp_avg", "exp_avg_sq"):
                 for name, start in ((key, at), (key + "_scale", at // BLOCK)) if packed else ((key, at),):
@@ -196,10 +197,10 @@ class ClipAdamW8(torch.optim.Optimizer):
                         exp_avg_sq_scale=b["exp_avg_sq_scale"].as_strided((blocks,), (1,), at // BLOCK))
         return dict(exp_avg=b["exp_avg_32"].as_strided(p.shape, p.stride(), at), exp_avg_sq=b["exp_avg_sq_32"].as_strided(p.shape, p.stride(), at))
 
-    def _give_state(self, p, count):
+    def _give_state(self, p, count, draw):
         t = self._index[p]
-        self._counts[t] = count
-        self.state[p] = dict(step=self._counts[t], **self._views(p))
+        self._counts[t], self._draws[t] = count, draw
+        self.state[p] = dict(step=self._counts[t], draw=self._draws[t], **self._views(p))
 
     def state_buffers(self):
         """The buffers that hold all parameters' moments (each parameter's from a multiple of 256 elements on, in the order of the groups, zeros
@@ -237,7 +238,7 @@ class ClipAdamW8(torch.optim.Optimizer):
                 raise RuntimeError(f"ClipAdamW8: a parameter of {self._sizes[p]} elements has {p.numel()} now (its moments have not)")
             st = self.state[p]
             if "exp_avg" not in st:
-                self._give_state(p, 0.0)
+                self._give_state(p, 0.0, 0)
             elif not _same_layout(st["exp_avg"], p):
                 raise RuntimeError("ClipAdamW8: a moment's layout differs from its parameter's")
         total = sum(p.numel() for p in ps)
@@ -266,7 +267,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         group_of = {p: gi for gi, g in enumerate(self.param_groups) for p in g["params"]}
         self._plan = dict(ps=ps, addresses=addresses, n_chunks=n_chunks, chunk=chunk, table=torch.from_numpy(table).to(dev),
                           chunk_t=torch.from_numpy(chunk_t).to(dev), chunk_o=torch.from_numpy(chunk_o).to(dev), slots=slots, turn=0,
-                          index=torch.tensor([self._index[p] for p in ps]), group=np.array([group_of[p] for p in ps]),
+                          index=np.array([self._index[p] for p in ps]), group=np.array([group_of[p] for p in ps]),
                           dtypes=[p.dtype for p in ps], as_checked=None)
         torch.cuda.current_stream(dev).synchronize()          # (built on this stream, read on whichever stream a step runs on)
         return self._plan
@@ -309,13 +310,14 @@ class ClipAdamW8(torch.optim.Optimizer):
                 slot["event"].synchronize()                   # (the step that last used this slot: RING steps ago)
             rows = slot["rows"]
             rows["grad"] = list(map(_ADDRESS, grads))
-            counts = self._counts[plan["index"]] + 1
-            self._fill(rows["h"], plan["group"], counts.numpy())
+            all_counts, all_draws, index = self._counts.numpy(), self._draws.numpy(), plan["index"]
+            counts, draw = all_counts[index] + 1, int(all_draws[index].max()) + 1
+            self._fill(rows["h"], plan["group"], counts)
             slot["device"].copy_(slot["host"], non_blocking=True)
-            self._counts[plan["index"]] = counts
+            all_counts[index], all_draws[index] = counts, draw
             stream = torch.cuda.current_stream(dev)
             _lib.timed_call("clip_adamw8", "mmt_clip_adamw8_step", plan["n_chunks"], plan["chunk"], plan["chunk_t"].data_ptr(), plan["chunk_o"].data_ptr(),
-                            plan["table"].data_ptr(), slot["device"].data_ptr(), self._key(int(counts.max())), self.max_norm,
+                            plan["table"].data_ptr(), slot["device"].data_ptr(), self._key(draw), self.max_norm,
                             slot["partials"].data_ptr(), slot["norm"].data_ptr(), stream.cuda_stream)
             slot["event"] = slot["event"] or torch.cuda.Event()
             slot["event"].record(stream)
@@ -343,8 +345,8 @@ class ClipAdamW8(torch.optim.Optimizer):
                 replaced = True
         plan["as_checked"] = None if replaced else _as_now(ps + grads)
 
-    def _key(self, count):
-        return _mix((_mix(self.seed & 0xFFFFFFFF) + count) & 0xFFFFFFFF)
+    def _key(self, draw):
+        return _mix((_mix(self.seed & 0xFFFFFFFF) + draw) & 0xFFFFFFFF)
 
     def _fill(self, h, group, counts):
         """The 8 floats of every tensor: from its group's hyper-parameters and its own step count."""
@@ -378,6 +380,10 @@ class ClipAdamW8(torch.optim.Optimizer):
                 st = saved.get(k, {})
                 if "exp_avg" in st or "exp_avg_sq" in st:
                     loaded[p] = self._loaded(p, st)
+            # (a state that does not name its draws was rounded, if at all, by ones up to the largest step count)
+            drawn = int(max([0, *(st["step"] for st in loaded.values()), *(st["draw"] for st in loaded.values())]))
+            for st in loaded.values():
+                st["draw"] = drawn if st["draw"] < 0 else st["draw"]
             return {**sd, "state": {}}
 
         def install(_):                           # first of the post-hooks: the rest find the moments there
@@ -398,7 +404,7 @@ class ClipAdamW8(torch.optim.Optimizer):
                 raise ValueError(f"ClipAdamW8: a state without {key}")
             if key != "step" and tuple(st[key].shape) != tuple(p.shape):
                 raise ValueError(f"ClipAdamW8: {key} of shape {tuple(st[key].shape)} for a parameter of shape {tuple(p.shape)}")
-        return dict(step=float(st["step"]), **self._converted(p, st, "exp_avg"), **self._converted(p, st, "exp_avg_sq"))
+        return dict(step=float(st["step"]), draw=int(st.get("draw", -1)), **self._converted(p, st, "exp_avg"), **self._converted(p, st, "exp_avg_sq"))
 
     def _converted(self, p, st, key):
         """A saved moment in the form and memory order that this parameter keeps it in: {key: codes, key_scale: scales} or {key: fp32}."""
