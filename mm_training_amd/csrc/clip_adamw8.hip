@@ -338,9 +338,15 @@ struct Lane4 {
             bf16_t q[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                // (bits + 16 random ones: an infinity stays one, and a NaN, whose low half is 0 where all that it can come from is bf16)
+                // (bits + 16 random ones: an infinity stays one)
                 if (BF16) q[j] = (bf16_t)((__float_as_uint(p[j]) + ((hash[j] * 0x6A09E667u) >> 16)) >> 16);
                 else q[j] = (bf16_t)(pack_bf16x2(p[j], 0.f) & 0xFFFFu);
+            }
+            // A NaN with ones in its low half (from an fp32 gradient through the norm, from an fp32 moment) could be carried past the largest pattern, into 0:
+            // it is made the quiet one.  Two comparisons for the four elements.
+            if (BF16 && (__builtin_isunordered(p[0], p[1]) || __builtin_isunordered(p[2], p[3]))) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q[j] = p[j] != p[j] ? (bf16_t)0x7FC0 : q[j];
             }
             const Global<bf16_t> to = global<bf16_t>(BF16 ? t.param : t.shadow) + i;
             if (WHOLE || i + 4 <= end) {
