@@ -916,7 +916,7 @@ int mmt_moment_unpack(int64_t n, const void *codes, const void *scales, int seco
  *            1 - beta2, 1 / sqrt(1 - beta2^t), eps -- every tensor has its own, so groups and step counts may differ
  *   chunk_tensor int32, chunk_offset int64 [num_chunks], DEVICE: chunks of chunk_elems elements (a multiple of 256), the offsets multiples of it
  *   key      random key of this step; max_norm <= 0: no clipping and no norm launch
- *   partials double [mmt_clip_adamw8_partials(num_chunks)] scratch; norm_out fp32 [2]: total norm over all tensors (summed in 64 bits), coefficient
+ *   partials double [mmt_clip_adamw8_partials(num_chunks)] scratch; norm_out fp32 [2]: total norm over all tensors (summed in 64 bits), coefficient; 0, 1 without clipping
  * With fp32 arithmetic in this order (no contraction): g = grad * coefficient; m = b1 m + (1 - b1) g; v = b2 v + ((1 - b2) g) g;
  * p = p * (1 - lr wd) - (m * step_size) / (sqrt(v) / sqrt(bc2) + eps).  The parameter takes m and v as they are; then their 8-bit codes
  * round them stochastically: 16 random bits are added to the part that is cut off.  The bits are h >> 16 (first moment) and h & 0xFFFF

@@ -91,7 +91,8 @@ class ClipAdamW8(torch.optim.Optimizer):
     leaves.  (Parameters that have taken part in every step: the step count.)
 
     ``state_dict()`` resumes exactly (with the same ``seed``).  ``load_state_dict`` also takes the state of torch.optim.AdamW or ClipAdamW (32-bit moments are packed), and
-    ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of the last step on the device.
+    ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of the last step on the device, a tensor of that step's
+    own; (0, 1) without clipping, which takes no norm.
     ``step()`` cannot be captured into a graph (gradients' addresses and step counts travel from the host): it raises."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=0.0, seed=0, min_8bit_size=4096):
@@ -262,8 +263,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         for _ in range(RING):   # what a step writes before its kernels have run: the step that takes the slot next waits for its event
             host = torch.empty(len(ps) * STEP_ROW.itemsize, dtype=torch.uint8).pin_memory()
             slots.append(dict(host=host, rows=host.numpy().view(STEP_ROW), device=torch.empty(host.numel(), dtype=torch.uint8, device=dev),
-                              partials=torch.empty(partials, dtype=torch.float64, device=dev),
-                              norm=torch.zeros(2, dtype=torch.float32, device=dev), event=None))
+                              partials=torch.empty(partials, dtype=torch.float64, device=dev), event=None))
         group_of = {p: gi for gi, g in enumerate(self.param_groups) for p in g["params"]}
         self._plan = dict(ps=ps, addresses=addresses, n_chunks=n_chunks, chunk=chunk, table=torch.from_numpy(table).to(dev),
                           chunk_t=torch.from_numpy(chunk_t).to(dev), chunk_o=torch.from_numpy(chunk_o).to(dev), slots=slots, turn=0,
@@ -315,14 +315,14 @@ class ClipAdamW8(torch.optim.Optimizer):
             self._fill(rows["h"], plan["group"], counts)
             slot["device"].copy_(slot["host"], non_blocking=True)
             all_counts[index], all_draws[index] = counts, draw
-            stream = torch.cuda.current_stream(dev)
+            stream, norm = torch.cuda.current_stream(dev), torch.empty(2, dtype=torch.float32, device=dev)
             _lib.timed_call("clip_adamw8", "mmt_clip_adamw8_step", plan["n_chunks"], plan["chunk"], plan["chunk_t"].data_ptr(), plan["chunk_o"].data_ptr(),
                             plan["table"].data_ptr(), slot["device"].data_ptr(), self._key(draw), self.max_norm,
-                            slot["partials"].data_ptr(), slot["norm"].data_ptr(), stream.cuda_stream)
+                            slot["partials"].data_ptr(), norm.data_ptr(), stream.cuda_stream)
             slot["event"] = slot["event"] or torch.cuda.Event()
             slot["event"].record(stream)
             plan["turn"] = (plan["turn"] + 1) % RING
-        self.last_norm = slot["norm"]
+        self.last_norm = norm
         return loss
 
     def _check_each(self, plan, ps, grads):
