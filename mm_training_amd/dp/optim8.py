@@ -170,6 +170,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._live = [p for p in ps if p.numel()]
         self._empty = [p for p in ps if not p.numel()]
         self._sizes = {p: p.numel() for p in ps}
+        torch.cuda.current_stream(dev).synchronize()          # (filled on this stream, stepped on whichever)
 
     def _fill_state(self, states):
         """The parameters' moments and step counts from other tensors of the same form, in the same memory order."""
@@ -268,7 +269,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._plan = dict(ps=ps, addresses=addresses, n_chunks=n_chunks, chunk=chunk, table=torch.from_numpy(table).to(dev),
                           chunk_t=torch.from_numpy(chunk_t).to(dev), chunk_o=torch.from_numpy(chunk_o).to(dev), slots=slots, turn=0,
                           index=np.array([self._index[p] for p in ps]), group=np.array([group_of[p] for p in ps]),
-                          dtypes=[p.dtype for p in ps], as_checked=None)
+                          dtypes=[p.dtype for p in ps], as_checked=None, streams=set())
         torch.cuda.current_stream(dev).synchronize()          # (built on this stream, read on whichever stream a step runs on)
         return self._plan
 
@@ -319,11 +320,20 @@ class ClipAdamW8(torch.optim.Optimizer):
             _lib.timed_call("clip_adamw8", "mmt_clip_adamw8_step", plan["n_chunks"], plan["chunk"], plan["chunk_t"].data_ptr(), plan["chunk_o"].data_ptr(),
                             plan["table"].data_ptr(), slot["device"].data_ptr(), self._key(draw), self.max_norm,
                             slot["partials"].data_ptr(), norm.data_ptr(), stream.cuda_stream)
+            if stream.cuda_stream not in plan["streams"]:
+                self._keep_for(stream, plan)
             slot["event"] = slot["event"] or torch.cuda.Event()
             slot["event"].record(stream)
             plan["turn"] = (plan["turn"] + 1) % RING
         self.last_norm = norm
         return loss
+
+    def _keep_for(self, stream, plan):
+        """What a step on this stream reads and writes keeps its memory until the stream is done with it, also when the optimizer is dropped before."""
+        plan["streams"].add(stream.cuda_stream)
+        for t in (*self._buffers.values(), *self.shadows.values(), plan["table"], plan["chunk_t"], plan["chunk_o"],
+                  *(slot[key] for slot in plan["slots"] for key in ("device", "partials"))):
+            t.record_stream(stream)
 
     def _check_each(self, plan, ps, grads):
         """Raises unless every parameter is laid out like its moments and has a dense gradient of its shape; gradients of another type or memory order
@@ -389,6 +399,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         def install(_):                           # first of the post-hooks: the rest find the moments there
             self._layout()                        # (new buffers: the given tensors may be views of the ones there were)
             self._fill_state(loaded)
+            torch.cuda.current_stream(self._buffers["exp_avg"].device).synchronize()
 
         hooks = self.register_load_state_dict_pre_hook(convert), self.register_load_state_dict_post_hook(install, prepend=True)
         try:
