@@ -243,6 +243,8 @@ class ClipAdamW8(torch.optim.Optimizer):
                 self._give_state(p, 0.0, 0)
             elif not _same_layout(st["exp_avg"], p):
                 raise RuntimeError("ClipAdamW8: a moment's layout differs from its parameter's")
+            if p in self.shadows and (p.dtype != torch.float32 or not _same_layout(self.shadows[p], p)):
+                raise RuntimeError("ClipAdamW8: a parameter's bf16 copy was made for another type or layout of it (make_bf16_shadows makes it anew)")
         total = sum(p.numel() for p in ps)
         chunk = self._chunk(total)
         table = np.zeros((len(ps), COLUMNS), dtype=np.int64)
