@@ -249,6 +249,14 @@ __device__ __forceinline__ unsigned reached_by(const unsigned *key, int want, in
     return lo;
 }
 
+// What lanes of a wave have written to LDS for one another, before they read it (or before they write the next): a wave's LDS operations are done in order,
+// so this only keeps the compiler from moving them.
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Alternatives of a row that a wave holds: the elements that reach the bound above side by side in the wave's lanes (two each at most), each counting the
 // ones in front of it.  false: more reach it (ties), nothing written.
 constexpr int kWaveCandidates = 128;
@@ -266,7 +274,7 @@ __device__ __forceinline__ bool wave_alternatives(const LogProbsArgs &a, int64_t
         if (key[i] >= lo) cand[at] = composite(key[i], x[i / N].s + i % N);
         base += __popcll(mask);
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_exchange();
     for (int i = lane; i < n; i += 64) {
         const unsigned long long own = cand[i];
         int rank = 0;
@@ -277,7 +285,7 @@ __device__ __forceinline__ bool wave_alternatives(const LogProbsArgs &a, int64_t
             a.top_log_prob[r * a.top + rank] = res.log_prob(key_value((unsigned)(own >> 32)));
         }
     }
-    __builtin_amdgcn_wave_barrier();
+    wave_exchange();
     return true;
 }
 
