@@ -20,6 +20,7 @@ BLOCK = 32          # elements that share a scale byte
 ALIGN = 256         # every tensor's moments begin at a multiple of this many elements of the state buffers
 COLUMNS = 9         # MMT_ADAMW8_COLUMNS
 _GRAD, _ADDRESS, _NUMEL = operator.attrgetter("grad"), torch.Tensor.data_ptr, torch.Tensor.numel           # (for map: a step asks every parameter)
+_PARAMS = operator.itemgetter("params")
 STEP_ROW = np.dtype([("grad", "<i8"), ("h", "<f4", (8,))])
 
 
@@ -33,6 +34,11 @@ def _mix(x):
 
 def _codes_dtype(second):
     return torch.float8_e5m2 if second else torch.float8_e4m3fn
+
+
+def _identical(a, b):
+    """The same objects in the same order."""
+    return len(a) == len(b) and all(map(operator.is_, a, b))
 
 
 def _as_now(tensors):
@@ -93,6 +99,8 @@ class ClipAdamW8(torch.optim.Optimizer):
     ``state_dict()`` resumes exactly (with the same ``seed``).  ``load_state_dict`` also takes the state of torch.optim.AdamW or ClipAdamW (32-bit moments are packed), and
     ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of the last step on the device, a tensor of that step's
     own; (0, 1) without clipping, which takes no norm.
+    The moments in ``state`` are views of ``state_buffers()``: to change them, write into them or load a state.  An entry that is taken out begins anew.
+    Parameters join by ``add_param_group`` only.
     ``step()`` cannot be captured into a graph (gradients' addresses and step counts travel from the host): it raises."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=0.0, seed=0, min_8bit_size=4096):
@@ -170,6 +178,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._live = [p for p in ps if p.numel()]
         self._empty = [p for p in ps if not p.numel()]
         self._sizes = {p: p.numel() for p in ps}
+        self._group_sizes = [len(g["params"]) for g in self.param_groups]
         torch.cuda.current_stream(dev).synchronize()          # (filled on this stream, stepped on whichever)
 
     def _fill_state(self, states):
@@ -233,6 +242,7 @@ class ClipAdamW8(torch.optim.Optimizer):
     def _tables(self, ps, addresses, grads):
         self._drop_plan()
         dev = self._buffers["exp_avg"].device
+        drawn = self._draws.numpy()
         for p, g in zip(ps, grads):                           # (everything but the gradients' addresses is read from the tables until these change)
             if p.device != dev or g.device != dev or p.dtype not in (torch.float32, torch.bfloat16) or not _dense(p):
                 raise TypeError(f"ClipAdamW8: a parameter is no longer a dense fp32 / bf16 one on {dev}, or its gradient is elsewhere")
@@ -240,7 +250,13 @@ class ClipAdamW8(torch.optim.Optimizer):
                 raise RuntimeError(f"ClipAdamW8: a parameter of {self._sizes[p]} elements has {p.numel()} now (its moments have not)")
             st = self.state[p]
             if "exp_avg" not in st:
-                self._give_state(p, 0.0, 0)
+                t = self._index[p]
+                if drawn[t]:                                  # (it had a state, which the program took out: zeros again, but no bits of the steps before)
+                    for x in self._views(p).values():
+                        x.view(torch.uint8).zero_() if x.element_size() == 1 else x.zero_()
+                self._give_state(p, 0.0, int(drawn[t]))
+            elif st["exp_avg"].data_ptr() != self._views(p)["exp_avg"].data_ptr():
+                raise RuntimeError("ClipAdamW8: a parameter's state was replaced by tensors that are not this optimizer's (load_state_dict takes them)")
             elif not _same_layout(st["exp_avg"], p):
                 raise RuntimeError("ClipAdamW8: a moment's layout differs from its parameter's")
             if p in self.shadows and (p.dtype != torch.float32 or not _same_layout(self.shadows[p], p)):
@@ -271,7 +287,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._plan = dict(ps=ps, addresses=addresses, n_chunks=n_chunks, chunk=chunk, table=torch.from_numpy(table).to(dev),
                           chunk_t=torch.from_numpy(chunk_t).to(dev), chunk_o=torch.from_numpy(chunk_o).to(dev), slots=slots, turn=0,
                           index=np.array([self._index[p] for p in ps]), group=np.array([group_of[p] for p in ps]),
-                          dtypes=[p.dtype for p in ps], as_checked=None, streams=set())
+                          dtypes=[p.dtype for p in ps], states=list(self.state.values()), as_checked=None, streams=set())
         torch.cuda.current_stream(dev).synchronize()          # (built on this stream, read on whichever stream a step runs on)
         return self._plan
 
@@ -293,26 +309,34 @@ class ClipAdamW8(torch.optim.Optimizer):
         with _lib.on_device(dev):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("ClipAdamW8.step() cannot be captured into a graph: gradients' addresses and step counts come from the host")
+        groups = list(map(_PARAMS, self.param_groups))
+        if list(map(len, groups)) != self._group_sizes or not all(map(operator.is_, itertools.chain.from_iterable(groups), self._params)):
+            raise RuntimeError("ClipAdamW8: the groups' parameters are not the ones that state was laid out for (add_param_group adds some; for others make a "
+                               "new optimizer and load the state)")
         ps = self._live
         grads = list(map(_GRAD, ps))
-        if any(map(operator.is_, grads, itertools.repeat(None))):          # (a parameter without a gradient takes no part)
+        try:
+            given = list(map(_ADDRESS, grads))
+        except (TypeError, RuntimeError):                     # (a parameter without a gradient takes no part; one without storage is refused below)
             ps = [p for p, g in zip(ps, grads) if g is not None]
-            grads = [g for g in grads if g is not None]
+            grads, given = [g for g in grads if g is not None], None
         if not ps:
             return loss
         addresses = list(map(_ADDRESS, ps))
         plan = self._plan
-        if plan is None or plan["addresses"] != addresses or not (plan["ps"] is ps or all(map(operator.is_, plan["ps"], ps))):
+        if (plan is None or plan["addresses"] != addresses or not (plan["ps"] is ps or _identical(plan["ps"], ps))
+                or not _identical(plan["states"], self.state.values())):
             plan = self._tables(ps, addresses, grads)
         # one question for all: is everything as it was when each was last looked at
         if plan["as_checked"] is None or not plan["as_checked"].check(*ps, *grads):
             self._check_each(plan, ps, grads)
+            given = None
         with _lib.on_device(dev):
             slot = plan["slots"][plan["turn"]]
             if slot["event"] is not None:
                 slot["event"].synchronize()                   # (the step that last used this slot: RING steps ago)
             rows = slot["rows"]
-            rows["grad"] = list(map(_ADDRESS, grads))
+            rows["grad"] = given or list(map(_ADDRESS, grads))
             all_counts, all_draws, index = self._counts.numpy(), self._draws.numpy(), plan["index"]
             counts, draw = all_counts[index] + 1, int(all_draws[index].max()) + 1
             self._fill(rows["h"], plan["group"], counts)
