@@ -14,7 +14,8 @@ import torch
 from torch._C._dynamo.guards import TensorGuards
 
 from .. import _lib
-from .optim import RING, _dense, _same_layout
+from .optim import RING, _dense
+from .optim import _same_layout as _same_order
 
 BLOCK = 32          # elements that share a scale byte
 ALIGN = 256         # every tensor's moments begin at a multiple of this many elements of the state buffers
@@ -34,6 +35,10 @@ def _mix(x):
 
 def _codes_dtype(second):
     return torch.float8_e5m2 if second else torch.float8_e4m3fn
+
+
+def _same_layout(a, b):
+    return a.stride() == b.stride() and a.shape == b.shape or _same_order(a, b)
 
 
 def _identical(a, b):
@@ -171,8 +176,11 @@ class ClipAdamW8(torch.optim.Optimizer):
         buffers = dict(exp_avg=u8(n8), exp_avg_scale=u8(n8 // BLOCK), exp_avg_sq=u8(n8), exp_avg_sq_scale=u8(n8 // BLOCK),
                        exp_avg_32=f32(n32), exp_avg_sq_32=f32(n32))
         self._buffers, self._place, self._params, self._n8 = buffers, place, ps, n8
+        self._bases = {key: t.data_ptr() for key, t in buffers.items()}
         self._typed = dict(buffers, exp_avg=buffers["exp_avg"].view(torch.float8_e4m3fn), exp_avg_sq=buffers["exp_avg_sq"].view(torch.float8_e5m2))
-        self._counts, self._draws = torch.zeros(len(ps), dtype=torch.float32), torch.zeros(len(ps), dtype=torch.int64)
+        counts, draws = torch.zeros(len(ps), dtype=torch.float32), torch.zeros(len(ps), dtype=torch.int64)
+        self._counts, self._draws = counts.numpy(), draws.numpy()             # (the same memory: the states' tensors are views of it)
+        self._count_of, self._draw_of = counts.unbind(), draws.unbind()
         self._index = {p: t for t, p in enumerate(ps)}
         self._fill_state(held)
         self._live = [p for p in ps if p.numel()]
@@ -208,10 +216,15 @@ class ClipAdamW8(torch.optim.Optimizer):
                         exp_avg_sq_scale=b["exp_avg_sq_scale"].as_strided((blocks,), (1,), at // BLOCK))
         return dict(exp_avg=b["exp_avg_32"].as_strided(p.shape, p.stride(), at), exp_avg_sq=b["exp_avg_sq_32"].as_strided(p.shape, p.stride(), at))
 
+    def _address(self, p):
+        """Where a parameter's first moment begins."""
+        packed, at = self._place[p]
+        return self._bases["exp_avg"] + at if packed else self._bases["exp_avg_32"] + 4 * at
+
     def _give_state(self, p, count, draw):
         t = self._index[p]
         self._counts[t], self._draws[t] = count, draw
-        self.state[p] = dict(step=self._counts[t], draw=self._draws[t], **self._views(p))
+        self.state[p] = dict(step=self._count_of[t], draw=self._draw_of[t], **self._views(p))
 
     def state_buffers(self):
         """The buffers that hold all parameters' moments (each parameter's from a multiple of 256 elements on, in the order of the groups, zeros
@@ -242,7 +255,6 @@ class ClipAdamW8(torch.optim.Optimizer):
     def _tables(self, ps, addresses, grads):
         self._drop_plan()
         dev = self._buffers["exp_avg"].device
-        drawn = self._draws.numpy()
         for p, g in zip(ps, grads):                           # (everything but the gradients' addresses is read from the tables until these change)
             if p.device != dev or g.device != dev or p.dtype not in (torch.float32, torch.bfloat16) or not _dense(p):
                 raise TypeError(f"ClipAdamW8: a parameter is no longer a dense fp32 / bf16 one on {dev}, or its gradient is elsewhere")
@@ -251,11 +263,11 @@ class ClipAdamW8(torch.optim.Optimizer):
             st = self.state[p]
             if "exp_avg" not in st:
                 t = self._index[p]
-                if drawn[t]:                                  # (it had a state, which the program took out: zeros again, but no bits of the steps before)
+                if self._draws[t]:                            # (it had a state, which the program took out: zeros again, but no bits of the steps before)
                     for x in self._views(p).values():
                         x.view(torch.uint8).zero_() if x.element_size() == 1 else x.zero_()
-                self._give_state(p, 0.0, int(drawn[t]))
-            elif st["exp_avg"].data_ptr() != self._views(p)["exp_avg"].data_ptr():
+                self._give_state(p, 0.0, int(self._draws[t]))
+            elif st["exp_avg"].data_ptr() != self._address(p):
                 raise RuntimeError("ClipAdamW8: a parameter's state was replaced by tensors that are not this optimizer's (load_state_dict takes them)")
             elif not _same_layout(st["exp_avg"], p):
                 raise RuntimeError("ClipAdamW8: a moment's layout differs from its parameter's")
@@ -264,7 +276,7 @@ class ClipAdamW8(torch.optim.Optimizer):
         total = sum(p.numel() for p in ps)
         chunk = self._chunk(total)
         table = np.zeros((len(ps), COLUMNS), dtype=np.int64)
-        base = {key: t.data_ptr() for key, t in self._buffers.items()}
+        base = self._bases
         for t, p in enumerate(ps):
             packed, at = self._place[p]
             if packed:
@@ -337,11 +349,11 @@ class ClipAdamW8(torch.optim.Optimizer):
                 slot["event"].synchronize()                   # (the step that last used this slot: RING steps ago)
             rows = slot["rows"]
             rows["grad"] = given or list(map(_ADDRESS, grads))
-            all_counts, all_draws, index = self._counts.numpy(), self._draws.numpy(), plan["index"]
-            counts, draw = all_counts[index] + 1, int(all_draws[index].max()) + 1
+            index = plan["index"]
+            counts, draw = self._counts[index] + 1, int(self._draws[index].max()) + 1
             self._fill(rows["h"], plan["group"], counts)
             slot["device"].copy_(slot["host"], non_blocking=True)
-            all_counts[index], all_draws[index] = counts, draw
+            self._counts[index], self._draws[index] = counts, draw
             stream, norm = torch.cuda.current_stream(dev), torch.empty(2, dtype=torch.float32, device=dev)
             _lib.timed_call("clip_adamw8", "mmt_clip_adamw8_step", plan["n_chunks"], plan["chunk"], plan["chunk_t"].data_ptr(), plan["chunk_o"].data_ptr(),
                             plan["table"].data_ptr(), slot["device"].data_ptr(), self._key(draw), self.max_norm,
