@@ -920,8 +920,8 @@ int mmt_moment_unpack(int64_t n, const void *codes, const void *scales, int seco
  * With fp32 arithmetic in this order (no contraction): g = grad * coefficient; m = b1 m + (1 - b1) g; v = b2 v + ((1 - b2) g) g;
  * p = p * (1 - lr wd) - (m * step_size) / (sqrt(v) / sqrt(bc2) + eps).  The parameter takes m and v as they are; then their 8-bit codes
  * round them stochastically: 16 random bits are added to the part that is cut off.  The bits are h >> 16 (first moment) and h & 0xFFFF
- * (second), h a 32-bit mix of (position + element + key) mod 2^32; a bf16 parameter takes the high half of another.  The same
- * inputs give the same bits; no atomics. */
+ * (second), h a 32-bit mix of (position + element + key) mod 2^32; a bf16 parameter takes the high half of another, and a NaN stays
+ * one.  The same inputs give the same bits; no atomics. */
 #define MMT_ADAMW8_COLUMNS 9
 int mmt_clip_adamw8_partials(int num_chunks);
 int mmt_clip_adamw8_step(int num_chunks, int chunk_elems, const int32_t *chunk_tensor, const int64_t *chunk_offset, const int64_t *tensors,

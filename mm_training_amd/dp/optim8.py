@@ -94,18 +94,22 @@ class ClipAdamW8(torch.optim.Optimizer):
     """AdamW with decoupled weight decay and ``clip_grad_norm_`` to ``max_norm`` (the norm over ALL groups; 0: no clipping) over dense fp32 / bf16
     CUDA parameters of one device.
 
-    State of a parameter: ``step`` and, from min_8bit_size elements on, ``exp_avg`` (float8_e4m3fn), ``exp_avg_sq`` (float8_e5m2) in the
-    parameter's shape and memory order with ``exp_avg_scale``, ``exp_avg_sq_scale`` (uint8 per 32 elements, see pack_moment); fp32 moments
-    below.  The update itself uses unrounded moments; what is stored is rounded stochastically by bits that are a function of ``seed``, the
-    element's position and the step's draw: one more than the largest that any parameter taking part has had (``draw`` in its state), so a run repeats
-    exactly, ranks of a data-parallel job agree, and a parameter never meets the bits of an earlier step again, whoever joins or
-    leaves.  (Parameters that have taken part in every step: the step count.)
+    State of a parameter: ``step``, ``draw`` and, from min_8bit_size elements on, ``exp_avg`` (float8_e4m3fn), ``exp_avg_sq`` (float8_e5m2) in
+    the parameter's shape and memory order with ``exp_avg_scale``, ``exp_avg_sq_scale`` (uint8 per 32 elements, see pack_moment); fp32
+    moments below.  The moments are views of ``state_buffers()``: to change them, write into them or load a state.  An entry that is
+    taken out begins anew.  Parameters join by ``add_param_group`` only.
 
-    ``state_dict()`` resumes exactly (with the same ``seed``).  ``load_state_dict`` also takes the state of torch.optim.AdamW or ClipAdamW (32-bit moments are packed), and
-    ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of the last step on the device, a tensor of that step's
-    own; (0, 1) without clipping, which takes no norm.
-    The moments in ``state`` are views of ``state_buffers()``: to change them, write into them or load a state.  An entry that is taken out begins anew.
-    Parameters join by ``add_param_group`` only.
+    The update itself uses unrounded moments; what is stored is rounded stochastically by bits that are a function of ``seed``, the element's
+    position and the step's draw: one more than the largest that any parameter taking part has had (``draw``; the step count where all
+    have taken part in every step).  So a run repeats exactly, ranks of a data-parallel job agree, and a parameter never meets the bits of
+    an earlier step again, whoever joins or leaves.
+
+    A gradient that is infinite or NaN makes NaN of the moments of the 32 elements that share its scale, for good; a NaN under clipping, through
+    the norm, of everything.
+
+    ``state_dict()`` resumes exactly (with the same ``seed``).  ``load_state_dict`` also takes the state of torch.optim.AdamW or ClipAdamW
+    (32-bit moments are packed), and ``state_dict_32bit()`` hands one to them.  ``last_norm`` holds (total norm, clip coefficient) of
+    the last step on the device, a tensor of that step's own; (0, 1) without clipping, which takes no norm.
     ``step()`` cannot be captured into a graph (gradients' addresses and step counts travel from the host): it raises."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_norm=0.0, seed=0, min_8bit_size=4096):

@@ -185,8 +185,8 @@ class TrainStep(nn.Module):
                     for t in list(self.model.parameters()) + list(self.model.buffers()):
                         dist.broadcast(t, 0)
             # Where the buckets are packed and the collectives issued: behind the weight gradients on THEIR stream (default), or on a
-            # stream of the reducer's own at normal priority (MMT_REDUCER_STREAM=own).  The review of round 4 asked for the latter
-            # (a collective queued behind a low-priority stream's backlog starts late); measured on ONE rank over RCCL
+            # stream of the reducer's own (MMT_REDUCER_STREAM=own): there a collective does not wait for the weight gradients' backlog.  Measured on
+            # ONE rank over RCCL, when the weight gradients' stream still had a lower priority than the others
             # (profiles/r05_exchange_tax.txt) the extra stream costs the rank 4.2 ms of a 66.7 ms step against 0.9 ms on the
             # weight-gradient stream -- a process has four hardware queues, and main + weight gradients + a communication
             # stream + RCCL's own are a fifth stream's worth of multiplexing.  What bounds the exposed tail instead is the size of
