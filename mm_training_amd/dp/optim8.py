@@ -159,8 +159,10 @@ class ClipAdamW8(torch.optim.Optimizer):
         self._check_params(ps)
         for g in self.param_groups:
             self._check_hyper(g)
-        held = {p: st for p, st in self.state.items() if "exp_avg" in st}
+        held, mine = {p: st for p, st in self.state.items() if "exp_avg" in st}, set(ps)
         for p, st in held.items():
+            if p not in mine or "draw" not in st:
+                raise RuntimeError("ClipAdamW8: a state is of a parameter that is in no group, or was put there directly (load_state_dict takes states)")
             if not _same_layout(st["exp_avg"], p) or ("exp_avg_scale" in st) != self._packed(p):
                 raise RuntimeError("ClipAdamW8: a parameter has changed its size or layout, and its moments (or min_8bit_size) have not")
         n8 = n32 = 0
@@ -424,11 +426,11 @@ class ClipAdamW8(torch.optim.Optimizer):
             saved = sd["state"]
             for g in sd["param_groups"]:
                 self._check_hyper({**self.defaults, **g})
-            order = [k for g in sd["param_groups"] for k in g["params"]]
-            if len(order) != len(self._params):
+            order, ps = ([p for g in groups for p in g["params"]] for groups in (sd["param_groups"], self.param_groups))
+            if len(order) != len(ps):
                 raise ValueError("ClipAdamW8: the state is of another number of parameters")
-            self._check_params(self._params)
-            for k, p in zip(order, self._params):
+            self._check_params(ps)
+            for k, p in zip(order, ps):
                 st = saved.get(k, {})
                 if "exp_avg" in st or "exp_avg_sq" in st:
                     loaded[p] = self._loaded(p, st)

@@ -108,3 +108,32 @@ def test_a_sparse_gradient_is_refused(mmt_lib):
     ps[1].grad = None
     opt.step()
     assert [int(opt.state[p]["step"]) for p in ps] == [2, 1, 2]
+
+
+def test_groups_edited_directly_then_laid_out_anew(mmt_lib):
+    """After a parameter was taken out of its group (or given a state directly) a further group is refused and does not stay; a loaded state lays everything out for
+    the parameters that are there."""
+    ps, opt = _go(2)
+    late = P(torch.ones(5000, device="cuda"))
+    gone = opt.param_groups[0]["params"].pop()
+    with pytest.raises(RuntimeError, match="ClipAdamW8"):
+        opt.add_param_group(dict(params=[late]))
+    assert len(opt.param_groups) == 1
+    del opt.state[gone]
+    given = {k: v.clone() for k, v in opt.state[ps[0]].items() if k != "draw"}
+    opt.state[late] = given
+    with pytest.raises(RuntimeError, match="ClipAdamW8"):
+        opt.add_param_group(dict(params=[late]))
+    assert len(opt.param_groups) == 1
+    del opt.state[late]
+    opt.load_state_dict(opt.state_dict())
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    before = gone.detach().clone()
+    opt.step()
+    assert torch.equal(gone, before) and [int(opt.state[p]["step"]) for p in ps[:2]] == [3, 3] and gone not in opt.state
+    twin_ps, twin = _go(2)
+    for p in twin_ps:
+        p.grad = torch.ones_like(p)
+    twin.step()
+    assert all(torch.equal(a, b) for a, b in zip(ps[:2], twin_ps[:2]))
